@@ -5,7 +5,7 @@
 //    collective scheduler (common/sched.hpp, the microcode analogue of
 //    reference ccl_offload_control.c) with the Cclo state staged in LDS;
 //    wave 1 is the inline small-mover (sub-32KB moves over an LDS mailbox).
-//  * accl_mover_kernel — the mover fleet (~10 of 16 wave slots per CU):
+//  * accl_mover_kernel — the mover fleet (171 workgroups of eight waves):
 //    static rotated tile partitioning, replicated packed doorbells,
 //    non-temporal software-pipelined copy / cast / n-ary reduce tiles
 //    between local HBM and peer HBM over xGMI (the data plane: reference
@@ -642,7 +642,11 @@ __device__ bool dtype_is_floatish(DataType d) {
 
 // Returns true if the executed path used only non-temporal accesses (no
 // dirty L2 lines -> the caller may skip the L2-writeback release fence).
-__device__ bool run_tile(const MoveDesc& m, u32 t, int lane) {
+// FLEET: for the mover kernel, whose registers are bounded; the scheduler's has
+// a copy of its own. Inlined it would keep addresses of every path in registers
+// and spill them.
+template <bool FLEET>
+__device__ __attribute__((noinline)) bool run_tile(const MoveDesc& m, u32 t, int lane) {
   u64 te = move_tile_elems(m);
   u64 lo = u64(t) * te;
   u64 hi = lo + te;
@@ -802,7 +806,8 @@ __device__ bool run_tile(const MoveDesc& m, u32 t, int lane) {
 // new move costs ~L2-hit latency, not a fleet-wide serialized cacheline.
 __device__ void mover_main(GpuEngineState* S) {
   const int lane = int(threadIdx.x) & 63;
-  const u32 gw = blockIdx.x * (blockDim.x / 64) + (threadIdx.x / 64);
+  // neighbouring waves, which get neighbouring tiles, are on different CUs
+  const u32 gw = (threadIdx.x / 64) * gridDim.x + blockIdx.x;
   const u32 nwaves = gridDim.x * (blockDim.x / 64);
   MoveDesc* ring = S->mover.ring;
   MoveState* st = S->mover.st;
@@ -875,7 +880,8 @@ __device__ void mover_main(GpuEngineState* S) {
         }
         if (lane == 0 && first == 0) S->dbg[1] = wallclock();
         u32 cnt = 0;
-        for (u32 t = first; t < total; t += nwaves, ++cnt) run_tile(m, t, lane);
+        for (u32 t = first; t < total; t += nwaves, ++cnt)
+          run_tile<true>(m, t, lane);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "");
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -989,7 +995,7 @@ __device__ void small_mover(SmallMb* mb, int lane) {
       __builtin_amdgcn_s_sleep(1);
       continue;
     }
-    bool nt = run_tile(mb->d, 0, lane);  // a small move fits one tile
+    bool nt = run_tile<false>(mb->d, 0, lane);  // a small move fits one tile
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if (!nt) {
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "");
@@ -1003,9 +1009,9 @@ __device__ void small_mover(SmallMb* mb, int lane) {
 }
 
 // Two kernels: the scheduler WG (control wave + small-mover wave — one CU)
-// and the mover fleet (lean copy/reduce waves, ~10 of the 16 wave slots
-// per CU so co-resident compute kernels always have room — config 5).
-__global__ void __launch_bounds__(128, 1) accl_scheduler_kernel(GpuEngineState* S) {
+// and the mover fleet. Each leaves half of a compute unit's registers to others,
+// and the bounds here are what keeps them to it (see gpu_engine_launch).
+__global__ void __launch_bounds__(128, 2) accl_scheduler_kernel(GpuEngineState* S) {
   __shared__ SmallMb mb;
   __shared__ Cclo<GpuMover> C;
   // the per-workgroup LDS budget on CDNA is 64 KB: exceeding it makes the
@@ -1032,7 +1038,7 @@ __global__ void __launch_bounds__(128, 1) accl_scheduler_kernel(GpuEngineState* 
   }
 }
 
-__global__ void __launch_bounds__(256, 2) accl_mover_kernel(GpuEngineState* S) {
+__global__ void __launch_bounds__(MOVER_THREADS, 4) accl_mover_kernel(GpuEngineState* S) {
   // bring-up telemetry: count mover WGs that actually started (dbg[15])
   if (threadIdx.x == 0)
     __hip_atomic_fetch_add(&S->dbg[15], 1ull, __ATOMIC_RELAXED,
@@ -1064,14 +1070,20 @@ void gpu_probe_launch(const ProbeArgs& a, void* stream) {
                      (hipStream_t)stream, a);
 }
 
-void gpu_scheduler_launch(GpuEngineState* state_dev, void* sched_stream) {
-  hipLaunchKernelGGL(accl_scheduler_kernel, dim3(1), dim3(128), 0,
-                     (hipStream_t)sched_stream, state_dev);
-}
-
-void gpu_mover_launch(GpuEngineState* state_dev, int n_wgs, void* mover_stream) {
-  hipLaunchKernelGGL(accl_mover_kernel, dim3(n_wgs), dim3(256), 0,
-                     (hipStream_t)mover_stream, state_dev);
+void gpu_engine_launch(GpuEngineState* state_dev, int n_groups, void* sched_stream,
+                       void* mover_stream) {
+  // both find room in either order (ACCL_MOVER_FIRST is for comparison)
+  if (std::getenv("ACCL_MOVER_FIRST")) {
+    hipLaunchKernelGGL(accl_mover_kernel, dim3(n_groups), dim3(MOVER_THREADS), 0,
+                       (hipStream_t)mover_stream, state_dev);
+    hipLaunchKernelGGL(accl_scheduler_kernel, dim3(1), dim3(128), 0,
+                       (hipStream_t)sched_stream, state_dev);
+  } else {
+    hipLaunchKernelGGL(accl_scheduler_kernel, dim3(1), dim3(128), 0,
+                       (hipStream_t)sched_stream, state_dev);
+    hipLaunchKernelGGL(accl_mover_kernel, dim3(n_groups), dim3(MOVER_THREADS), 0,
+                       (hipStream_t)mover_stream, state_dev);
+  }
 }
 
 }  // namespace accl

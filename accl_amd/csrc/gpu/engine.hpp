@@ -92,15 +92,34 @@ struct GpuEngineState {
   u64 dbg[16];
 };
 
-// Launch the persistent engine kernels (defined in engine.hip). The scheduler
-// has to run before the mover fleet is launched: its waves need 376 registers,
-// and a fleet of 640 workgroups leaves at most 208 on every SIMD, so a fleet
-// that gets there first keeps the scheduler out for good. The order of two
-// launches on two streams does not decide that (the scheduler's queue may
-// still be waiting for its scratch memory): the host waits for engine_up in
-// between.
-void gpu_scheduler_launch(GpuEngineState* state_dev, void* sched_stream);
-void gpu_mover_launch(GpuEngineState* state_dev, int n_wgs, void* mover_stream);
+// Launches the persistent engine kernels (defined in engine.hip): scheduler on
+// sched_stream, n_groups mover workgroups on mover_stream.
+//
+// Neither kernel ends before shutdown, and a move waits for the waves that own
+// its tiles, so all of them have to be resident together, also with engines of
+// other processes on the same GPU and in whatever order they come: the driver
+// saves and places them anew whenever a process makes or drops a hardware queue.
+// The hardware deals workgroups out to the 32 shader engines of eight compute
+// units in turn and lets one wait if its engine is full, though others are not.
+// So neither kernel takes more than half of the 512 registers of a compute unit's
+// SIMDs (a scheduler's wave 256, a mover group two waves of 120 on each): any two
+// of these workgroups fit on a compute unit, a shader engine has 16 places, and a
+// fleet takes five or six of them.
+// A scheduler of 376 registers found no place beside a fleet of 640 workgroups of
+// four waves with 152 until that fleet ended, and with movers that fill a compute
+// unit (1024 threads) a shader engine was full now and then. One of 144 registers
+// was placed by each of three movers on its SIMD, for which moves then waited:
+// 16 MiB copied in 85 us instead of 68.
+constexpr int MOVER_THREADS = 512;
+constexpr int MOVER_GROUPS_MAX = 240;
+
+// Engines are sized by their users in quarters of a group.
+inline int mover_groups(int wgs) {
+  const int n = wgs / 4 + (wgs % 4 != 0);
+  return n < 1 ? 1 : n < MOVER_GROUPS_MAX ? n : MOVER_GROUPS_MAX;
+}
+void gpu_engine_launch(GpuEngineState* state_dev, int n_groups, void* sched_stream,
+                       void* mover_stream);
 
 // bring-up handshake probe (shader-store into every peer mapping)
 constexpr u64 PROBE_MAGIC = 0x50524F4245000000ull;  // "PROBE" | rank

@@ -286,14 +286,11 @@ void GpuDevice::connect(const std::vector<std::vector<char>>& blobs) {
   __atomic_store_n((u64*)&ring_->ctrl.comm_gen, 1, __ATOMIC_RELEASE);
 
   CSTAGE("state uploaded; launching engine");
-  // ACCL_MOVER_FIRST restores the old order for comparison
-  const bool mover_first = std::getenv("ACCL_MOVER_FIRST") != nullptr;
-  if (mover_first)
-    gpu_mover_launch((GpuEngineState*)state_dev_, engine_wgs_, mover_stream_);
-  gpu_scheduler_launch((GpuEngineState*)state_dev_, stream_);
+  gpu_engine_launch((GpuEngineState*)state_dev_, mover_groups(engine_wgs_),
+                    stream_, mover_stream_);
   hip_check(hipGetLastError(), "engine kernel launch");
   launched_ = true;
-  CSTAGE("scheduler launched; waiting engine_up");
+  CSTAGE("kernels launched; waiting engine_up");
   // wait for the engine to come up
   u64 t0 = wallclock_host_ns();
   while (!__atomic_load_n((u64*)&ring_->ctrl.engine_up, __ATOMIC_ACQUIRE)) {
@@ -305,15 +302,10 @@ void GpuDevice::connect(const std::vector<std::vector<char>>& blobs) {
                       sizeof(u64), hipMemcpyDeviceToHost);
       throw accl_error("gpu: engine kernel never came up (mover WGs "
                        "started: " + std::to_string(movers_started) + "/" +
-                       std::to_string(engine_wgs_) + ")");
+                       std::to_string(mover_groups(engine_wgs_)) + ")");
     }
     usleep(100);
   }
-  if (!mover_first) {
-    gpu_mover_launch((GpuEngineState*)state_dev_, engine_wgs_, mover_stream_);
-    hip_check(hipGetLastError(), "mover kernel launch");
-  }
-  CSTAGE("movers launched");
 }
 
 void GpuDevice::shutdown() {

@@ -48,9 +48,10 @@ class GpuDevice : public Backend {
 
  private:
   int dev_ = 0;
-  int engine_wgs_ = 640;  // 256-thr WGs, ~2.5 per CU (mover VGPR use caps
-                          // occupancy at 3 WGs/CU; wave slots and >70
-                          // VGPRs/SIMD stay free for co-resident kernels)
+  // Four make a mover group: 171 groups, of which the 512 tiles of a 256 MiB move
+  // are three for each (178 us; with 160 groups 190, with 192 180). Up to 1 MiB
+  // more groups only wake up later (64 KiB 32 us, with 192 35).
+  int engine_wgs_ = 684;
   u64 arena_bytes_ = 0;
   ArenaLayout layout_{};
   bool fine_grained_ = true;
