@@ -5,8 +5,10 @@
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 #include <cstring>
+#include <mutex>
 #include <unistd.h>
 #include "../core/accl.hpp"
+#include "../core/util.hpp"
 #include "../emu/emudevice.hpp"
 #include <hip/hip_runtime.h>
 #include "../gpu/gpudevice.hpp"
@@ -72,6 +74,35 @@ static py::capsule make_dlpack(BaseBuffer& b, bool gpu, int device_id) {
 }
 
 // ------------------------------------------------------------ module ----
+// A demo kernel on a stream of its own (the engine's streams hold kernels that
+// never end, so anything queued behind them would never run), waited for with a
+// bound. The kernels' own waits are bounded too; one that has not ended here was
+// never placed, and its stream stays, since to destroy it would wait for it.
+template <class Launch>
+static void run_demo(const char* what, GpuDevice* g, Launch&& launch) {
+  std::lock_guard<std::mutex> one_at_a_time(g->demo_mutex);
+  hipStream_t st{};
+  if (hipStreamCreateWithFlags(&st, hipStreamNonBlocking) != hipSuccess)
+    throw accl_error(std::string(what) + ": stream create failed");
+  volatile u32* err = g->demo_result();
+  *err = E_OK;
+  launch((u32*)err, st);
+  hipError_t e = hipGetLastError();
+  u64 t0 = wallclock_host_ns();
+  while (e == hipSuccess) {
+    hipError_t q = hipStreamQuery(st);
+    if (q != hipErrorNotReady) { e = q; break; }
+    if (wallclock_host_ns() - t0 > 30ull * 1000000000)
+      throw accl_error(std::string(what) + ": the kernel did not end");
+    usleep(100);
+  }
+  (void)hipStreamDestroy(st);
+  if (e != hipSuccess)
+    throw accl_error(std::string(what) + ": " + hipGetErrorString(e));
+  if (*err != E_OK)
+    throw accl_error(std::string(what) + ": " + error_to_string(*err));
+}
+
 PYBIND11_MODULE(_core, m) {
   m.doc() = "accl_amd core: MI355X-native ACCL-class collective engine";
 
@@ -578,67 +609,36 @@ PYBIND11_MODULE(_core, m) {
            u32 tag, float addv) {
           auto* g = dynamic_cast<GpuDevice*>(a.backend());
           if (!g) throw accl_error("demo_vadd_devicecall: gpu backend only");
-          hipStream_t st{};
-          if (hipStreamCreateWithFlags(&st, hipStreamNonBlocking) != hipSuccess)
-            throw accl_error("demo: stream create failed");
-          launch_vadd_devicecall(
-              g->arena_local() + src.arena_offset(),
-              g->arena_local() + scratch.arena_offset(),
-              scratch.arena_offset(), count, tag, g->arena_local(), dst, addv,
-              st);
-          hipError_t e = hipGetLastError();
-          u64 t0 = wallclock_host_ns();
-          while (e == hipSuccess) {
-            hipError_t q = hipStreamQuery(st);
-            if (q != hipErrorNotReady) { e = q; break; }
-            if (wallclock_host_ns() - t0 > 30ull * 1000000000) {
-              e = hipErrorUnknown;
-              break;
-            }
-            usleep(100);
-          }
-          (void)hipStreamDestroy(st);
-          if (e != hipSuccess)
-            throw accl_error(std::string("demo_vadd_devicecall: ") +
-                             hipGetErrorString(e));
+          run_demo("demo_vadd_devicecall", g, [&](u32* err, hipStream_t st) {
+            launch_vadd_devicecall(
+                g->arena_local() + src.arena_offset(),
+                g->arena_local() + scratch.arena_offset(),
+                scratch.arena_offset(), count, tag, g->arena_local(), dst, addv,
+                err, st);
+          });
         },
         py::arg("a"), py::arg("src"), py::arg("scratch"), py::arg("count"),
         py::arg("dst"), py::arg("tag") = 0, py::arg("addv") = 1.0f,
         py::call_guard<py::gil_scoped_release>());
 
-  // demo plugin: device-initiated stream_put (reference vadd_put analogue)
+  // demo plugin: device-initiated stream_put (reference vadd_put analogue).
+  // wait_ms: how long the kernel waits for room in the ring
   m.def("demo_vadd_put",
-        [](ACCL& a, BaseBuffer& src, u64 count, u32 dst, u32 tag, float addv) {
+        [](ACCL& a, BaseBuffer& src, u64 count, u32 dst, u32 tag, float addv,
+           u32 wait_ms) {
           auto* g = dynamic_cast<GpuDevice*>(a.backend());
           if (!g) throw accl_error("demo_vadd_put: gpu backend only");
           u32 seg = g->cfg().stream_bytes < (32u << 10) ? g->cfg().stream_bytes
                                                         : (32u << 10);
-          // fresh stream: the engine's streams hold never-ending persistent
-          // kernels, so anything queued behind them would never run
-          hipStream_t st{};
-          if (hipStreamCreateWithFlags(&st, hipStreamNonBlocking) != hipSuccess)
-            throw accl_error("demo_vadd_put: stream create failed");
-          launch_vadd_put(g->arena_local() + src.arena_offset(), count, tag,
-                          g->arena_local(), g->peer_base(dst), g->cfg().rank,
-                          dst, seg, addv, st);
-          hipError_t e = hipGetLastError();
-          u64 t0 = wallclock_host_ns();
-          while (e == hipSuccess) {  // bounded sync (30 s)
-            hipError_t q = hipStreamQuery(st);
-            if (q != hipErrorNotReady) { e = q; break; }
-            if (wallclock_host_ns() - t0 > 30ull * 1000000000) {
-              e = hipErrorUnknown;
-              break;
-            }
-            usleep(100);
-          }
-          (void)hipStreamDestroy(st);
-          if (e != hipSuccess)
-            throw accl_error(std::string("demo_vadd_put: ") +
-                             hipGetErrorString(e));
+          run_demo("demo_vadd_put", g, [&](u32* err, hipStream_t st) {
+            launch_vadd_put(g->arena_local() + src.arena_offset(), count, tag,
+                            g->arena_local(), g->peer_base(dst), g->cfg().rank,
+                            dst, seg, addv, u64(wait_ms) * 1000 * TICKS_PER_US,
+                            err, st);
+          });
         },
         py::arg("a"), py::arg("src"), py::arg("count"), py::arg("dst"),
-        py::arg("tag") = 0, py::arg("addv") = 1.0f,
+        py::arg("tag") = 0, py::arg("addv") = 1.0f, py::arg("wait_ms") = 10000,
         py::call_guard<py::gil_scoped_release>());
 
   register_tensor_ops(m);

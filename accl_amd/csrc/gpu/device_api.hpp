@@ -12,6 +12,11 @@
 //
 // All functions are WAVE-collective: call them from one 64-lane wavefront
 // (lane = threadIdx.x & 63); lane 0 performs the control-word traffic.
+//
+// No function waits without a bound: what a peer, a consumer or the engine does
+// not provide within wait_ticks (of 10 ns) is given up, and the call says so. A
+// call that gives up while it waits for room has taken nothing: the ring is as
+// it was for the next one.
 #pragma once
 #include <hip/hip_runtime.h>
 #include "../common/proto.hpp"
@@ -20,6 +25,10 @@ namespace accl {
 namespace device_api {
 
 #define ACCL_DEV_SYS __HIP_MEMORY_SCOPE_SYSTEM
+
+constexpr u64 WAIT_TICKS = 10ull * 1000 * 1000 * TICKS_PER_US;  // 10 s
+constexpr u32 POP_TIMEOUT = ~0u;      // stream_pop: nothing came
+constexpr u64 CALL_TIMEOUT = ~0ull;   // device_call: no room in the ring
 
 struct StreamChan {
   // channel (me -> peer): payload ring in the PEER's arena, credit +
@@ -58,27 +67,42 @@ __device__ inline StreamChan stream_chan(char* my_arena, char* peer_arena,
 }
 
 // Push one segment (bytes <= stream_bytes) into the peer's ring.
-// Wave-collective; returns the segment's sequence number.
+// Wave-collective; returns the segment's sequence number (from 1), or 0 if the
+// consumer left no room within wait_ticks.
 __device__ inline u64 stream_push(const StreamChan& c, const void* data,
-                                  u32 bytes, u32 tag, u32 msg_flags = SEG_FIRST | SEG_LAST) {
+                                  u32 bytes, u32 tag,
+                                  u32 msg_flags = SEG_FIRST | SEG_LAST,
+                                  u64 wait_ticks = WAIT_TICKS) {
   EagerChanCtl* ctl = (EagerChanCtl*)(c.my_arena + c.ctl_off_mine);
   const int lane = int(threadIdx.x) & 63;
   u64 seq = 0;
   if (lane == 0) {
-    // tx counter shared with the engine and the host
-    seq = __hip_atomic_fetch_add(&ctl->tx_ctr, 1ull, __ATOMIC_RELAXED,
-                                 ACCL_DEV_SYS) + 1;
-    // credit gate: slot free once consumer advanced past seq - n_stream
+    // the tx counter is shared with the engine and the host; a number is taken
+    // only once its slot is free, that is once the consumer advanced past it
     // (in-loop acquire: the consumer may be another process — see
     // stream_pop's staleness note)
-    while (__hip_atomic_load(&ctl->credit, __ATOMIC_RELAXED, ACCL_DEV_SYS) +
-               c.n_stream < seq) {
+    const u64 t0 = wallclock();
+    u64 sent = __hip_atomic_load(&ctl->tx_ctr, __ATOMIC_RELAXED, ACCL_DEV_SYS);
+    for (;;) {
+      if (__hip_atomic_load(&ctl->credit, __ATOMIC_RELAXED, ACCL_DEV_SYS) +
+              c.n_stream > sent) {
+        if (__hip_atomic_compare_exchange_strong(&ctl->tx_ctr, &sent, sent + 1,
+                                                 __ATOMIC_RELAXED,
+                                                 __ATOMIC_RELAXED, ACCL_DEV_SYS)) {
+          seq = sent + 1;
+          break;
+        }
+        continue;  // `sent` is what another producer made of it
+      }
+      if (wallclock() - t0 > wait_ticks) break;
       __builtin_amdgcn_s_sleep(8);
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "");
+      sent = __hip_atomic_load(&ctl->tx_ctr, __ATOMIC_RELAXED, ACCL_DEV_SYS);
     }
   }
   seq = u64(__shfl(int(seq & 0xFFFFFFFF), 0, 64)) |
         (u64(u32(__shfl(int(seq >> 32), 0, 64))) << 32);
+  if (seq == 0) return 0;
   u32 slot = u32((seq - 1) % c.n_stream);
   // payload: wave-cooperative copy into the peer slot over xGMI
   char* dst = c.peer_arena + c.pay_off_peer + u64(slot) * c.stream_bytes;
@@ -131,9 +155,11 @@ __device__ inline StreamRx stream_rx(char* my_arena, char* peer_arena,
 }
 
 // Pop the next segment (sequence `seq`, 1-based caller-tracked) into dst.
-// Wave-collective; returns payload bytes, fills *tag. Spins until arrival.
+// Wave-collective; returns payload bytes, fills *tag. Waits for its arrival, and
+// returns POP_TIMEOUT if that takes longer than wait_ticks.
 __device__ inline u32 stream_pop(const StreamRx& r, u64 seq, void* dst,
-                                 u32 max_bytes, u32* tag) {
+                                 u32 max_bytes, u32* tag,
+                                 u64 wait_ticks = WAIT_TICKS) {
   const int lane = int(threadIdx.x) & 63;
   u32 slot = u32((seq - 1) % r.n_stream);
   SlotHdr* h = (SlotHdr*)(r.my_arena + r.hdr_off_mine) + slot;
@@ -142,7 +168,10 @@ __device__ inline u32 stream_pop(const StreamRx& r, u64 seq, void* dst,
   // multi-wave workgroup — an s_barrier here would hang the sibling waves).
   // The in-loop acquire drops stale L2 lines: the producer may be another
   // PROCESS (IPC) whose stores do not invalidate this XCD's L2 copies.
+  const u64 t0 = wallclock();
   while (__hip_atomic_load(&h->seq, __ATOMIC_RELAXED, ACCL_DEV_SYS) != seq) {
+    // the clock is the wave's, so that all lanes give up together
+    if (wallclock() - t0 > wait_ticks) return POP_TIMEOUT;
     __builtin_amdgcn_s_sleep(8);
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "");
   }
@@ -169,24 +198,32 @@ __device__ inline u32 stream_pop(const StreamRx& r, u64 seq, void* dst,
 // A kernel enqueues a full collective on its OWN engine (the reference's
 // ACCLCommand::start_call path, driver/hls/accl_hls.h:134-188, arbitrated
 // with host calls like client_arbiter.cpp:21-51). Lane-0-only (call from
-// one lane or guard with lane==0); returns a token for device_call_wait.
-__device__ inline u64 device_call(char* my_arena, const CallDesc& d) {
+// one lane or guard with lane==0); returns a token for device_call_wait, or
+// CALL_TIMEOUT if the engine freed no slot within wait_ticks.
+__device__ inline u64 device_call(char* my_arena, const CallDesc& d,
+                                  u64 wait_ticks = WAIT_TICKS) {
   const ArenaHdr* h = (const ArenaHdr*)my_arena;
   DevCallRing* ring = (DevCallRing*)(my_arena + h->devcall_off);
-  u64 idx = __hip_atomic_fetch_add(&ring->head, 1ull, __ATOMIC_RELAXED,
-                                   ACCL_DEV_SYS);
-  DevCallSlot* s = (DevCallSlot*)((char*)ring + sizeof(DevCallRing)) +
-                   (idx % DEVCALL_RING);
-  // slot reuse guard: wait until the previous occupant's ret was published
-  if (idx >= DEVCALL_RING) {
-    DevCallRet* prev =
-        (DevCallRet*)((char*)ring + sizeof(DevCallRing) +
-                      u64(DEVCALL_RING) * sizeof(DevCallSlot)) +
-        (idx % DEVCALL_RING);
-    while (__hip_atomic_load(&prev->seq, __ATOMIC_RELAXED, ACCL_DEV_SYS) <
-           idx + 1 - DEVCALL_RING)
-      __builtin_amdgcn_s_sleep(16);
+  DevCallSlot* slots = (DevCallSlot*)((char*)ring + sizeof(DevCallRing));
+  DevCallRet* rets = (DevCallRet*)(slots + DEVCALL_RING);
+  const u64 t0 = wallclock();
+  u64 idx = __hip_atomic_load(&ring->head, __ATOMIC_RELAXED, ACCL_DEV_SYS);
+  for (;;) {
+    // a slot is free once its previous occupant's ret was published
+    if (idx < DEVCALL_RING ||
+        __hip_atomic_load(&rets[idx % DEVCALL_RING].seq, __ATOMIC_RELAXED,
+                          ACCL_DEV_SYS) >= idx + 1 - DEVCALL_RING) {
+      if (__hip_atomic_compare_exchange_strong(&ring->head, &idx, idx + 1,
+                                               __ATOMIC_RELAXED, __ATOMIC_RELAXED,
+                                               ACCL_DEV_SYS))
+        break;
+      continue;  // `idx` is what another kernel made of it
+    }
+    if (wallclock() - t0 > wait_ticks) return CALL_TIMEOUT;
+    __builtin_amdgcn_s_sleep(16);
+    idx = __hip_atomic_load(&ring->head, __ATOMIC_RELAXED, ACCL_DEV_SYS);
   }
+  DevCallSlot* s = slots + idx % DEVCALL_RING;
   s->d = d;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "");
@@ -195,15 +232,21 @@ __device__ inline u64 device_call(char* my_arena, const CallDesc& d) {
   return idx;
 }
 
-// Poll completion of a device_call; returns errcode (0 = OK). Blocking.
-__device__ inline u32 device_call_wait(char* my_arena, u64 token) {
+// Waits for a device_call; returns its errcode (0 = OK), or E_TIMEOUT if the
+// engine does not answer within wait_ticks. (The call may still be served.)
+__device__ inline u32 device_call_wait(char* my_arena, u64 token,
+                                       u64 wait_ticks = WAIT_TICKS) {
+  if (token == CALL_TIMEOUT) return E_TIMEOUT;
   const ArenaHdr* h = (const ArenaHdr*)my_arena;
   DevCallRing* ring = (DevCallRing*)(my_arena + h->devcall_off);
   DevCallRet* r = (DevCallRet*)((char*)ring + sizeof(DevCallRing) +
                                 u64(DEVCALL_RING) * sizeof(DevCallSlot)) +
                   (token % DEVCALL_RING);
-  while (__hip_atomic_load(&r->seq, __ATOMIC_RELAXED, ACCL_DEV_SYS) < token + 1)
+  const u64 t0 = wallclock();
+  while (__hip_atomic_load(&r->seq, __ATOMIC_RELAXED, ACCL_DEV_SYS) < token + 1) {
+    if (wallclock() - t0 > wait_ticks) return E_TIMEOUT;
     __builtin_amdgcn_s_sleep(16);
+  }
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "");
   return u32(r->errcode);
 }

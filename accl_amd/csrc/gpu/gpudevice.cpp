@@ -84,6 +84,7 @@ GpuDevice::GpuDevice(u32 nranks, u32 rank, int device_index,
   hip_check(hipHostMalloc(&ring_pinned_, sizeof(RingPage), 0), "hipHostMalloc ring");
   std::memset(ring_pinned_, 0, sizeof(RingPage));
   ring_ = (RingPage*)ring_pinned_;
+  hip_check(hipHostMalloc(&demo_pinned_, sizeof(u32), 0), "hipHostMalloc demo");
 
   hip_check(hipMalloc(&state_dev_, sizeof(GpuEngineState)), "hipMalloc state");
   hipStream_t s;
@@ -100,6 +101,7 @@ GpuDevice::~GpuDevice() {
   if (state_dev_) (void)hipFree(state_dev_);
   if (arena_base_) (void)hipFree(arena_base_);
   if (ring_pinned_) (void)hipHostFree(ring_pinned_);
+  if (demo_pinned_) (void)hipHostFree(demo_pinned_);
   if (stream_) (void)hipStreamDestroy((hipStream_t)stream_);
   if (mover_stream_) (void)hipStreamDestroy((hipStream_t)mover_stream_);
 }

@@ -7,20 +7,21 @@
 // driver/utils/accl_network_utils/ — POE configuration becomes IPC handle
 // exchange + peer mapping).
 #pragma once
+#include <mutex>
 #include "../core/backend.hpp"
 
 namespace accl {
 
-// plugin launchers (gpu/plugins.hip)
+// plugin launchers (gpu/plugins.hip); err: host memory that the kernel can write
 void launch_vadd_put(const void* in, u64 count, u32 tag, void* my_arena,
                      void* peer_arena, u32 me, u32 peer, u32 seg_bytes,
-                     float addv, void* stream);
+                     float addv, u64 wait_ticks, u32* err, void* stream);
 void launch_stream_drain(void* out, u64 max_elems, u32 nseg, void* my_arena,
                          void* peer_arena, u32 me, u32 peer, u64 start_seq,
                          void* stream);
 void launch_vadd_devicecall(const void* in, void* scratch, u64 scratch_off,
                             u64 count, u32 tag, void* my_arena, u32 dst_rank,
-                            float addv, void* stream);
+                            float addv, u32* err, void* stream);
 
 class GpuDevice : public Backend {
  public:
@@ -45,6 +46,10 @@ class GpuDevice : public Backend {
   std::vector<u64> debug_timeline();
   char* peer_base(u32 r) const { return r < MAX_RANKS ? peer_base_[r] : nullptr; }
   void* op_stream() const { return stream_; }  // for plugin launches
+  // where a plugin kernel leaves its error code: host memory of the device's own,
+  // since to free any while the engine runs would wait for the engine to end
+  u32* demo_result() const { return (u32*)demo_pinned_; }
+  std::mutex demo_mutex;
 
  private:
   int dev_ = 0;
@@ -58,6 +63,7 @@ class GpuDevice : public Backend {
   void* mover_stream_ = nullptr;
   char* peer_base_[MAX_RANKS] = {};
   void* ring_pinned_ = nullptr;     // RingPage, hipHostMalloc
+  void* demo_pinned_ = nullptr;     // u32, hipHostMalloc
   void* state_dev_ = nullptr;       // GpuEngineState, hipMalloc
   void* stream_ = nullptr;          // hipStream_t
   bool launched_ = false;

@@ -9,10 +9,11 @@
 
 namespace accl {
 
-// single-wave demo kernel: stage each segment in LDS, push over xGMI
+// single-wave demo kernel: stage each segment in LDS, push over xGMI. *err is
+// E_TIMEOUT if the consumer left no room for a segment within wait_ticks.
 __global__ void __launch_bounds__(64, 1) vadd_put_kernel(
     const float* in, u64 count, u32 tag, char* my_arena, char* peer_arena,
-    u32 me, u32 peer, u32 seg_bytes, float addv) {
+    u32 me, u32 peer, u32 seg_bytes, float addv, u64 wait_ticks, u32* err) {
   __shared__ float stage[8192];  // 32 KiB staging
   auto chan = device_api::stream_chan(my_arena, peer_arena, me, peer);
   const int lane = int(threadIdx.x) & 63;
@@ -22,7 +23,11 @@ __global__ void __launch_bounds__(64, 1) vadd_put_kernel(
     u32 n = u32(count - off < seg_elems ? count - off : seg_elems);
     for (u32 i = lane; i < n; i += 64) stage[i] = in[off + i] + addv;
     __syncthreads();  // LDS visibility within the wave/WG
-    device_api::stream_push(chan, stage, n * 4, tag);
+    if (!device_api::stream_push(chan, stage, n * 4, tag, SEG_FIRST | SEG_LAST,
+                                 wait_ticks)) {
+      if (lane == 0) *err = E_TIMEOUT;
+      return;
+    }
     __syncthreads();
   }
 }
@@ -36,6 +41,7 @@ __global__ void __launch_bounds__(64, 1) stream_drain_kernel(
   for (u32 s = 0; s < nseg; ++s) {
     u32 nb = device_api::stream_pop(
         rx, start_seq + s, out + done, u32((max_elems - done) * 4), nullptr);
+    if (nb == device_api::POP_TIMEOUT) return;
     done += nb / 4;
   }
 }
@@ -46,7 +52,7 @@ __global__ void __launch_bounds__(64, 1) stream_drain_kernel(
 // ACCLCommand::stream_put flow, arbitrated with host calls).
 __global__ void __launch_bounds__(64, 1) vadd_devicecall_kernel(
     const float* in, float* scratch_arena_buf, u64 scratch_off, u64 count,
-    u32 tag, char* my_arena, u32 dst_rank, float addv) {
+    u32 tag, char* my_arena, u32 dst_rank, float addv, u32* err) {
   const int lane = int(threadIdx.x) & 63;
   for (u64 i = lane; i < count; i += 64)
     scratch_arena_buf[i] = in[i] + addv;
@@ -65,26 +71,26 @@ __global__ void __launch_bounds__(64, 1) vadd_devicecall_kernel(
     d.addr0 = scratch_off;
     d.flags = F_SRC_ARENA;
     u64 tok = device_api::device_call(my_arena, d);
-    u32 e = device_api::device_call_wait(my_arena, tok);
-    (void)e;
+    *err = device_api::device_call_wait(my_arena, tok);
   }
 }
 
 void launch_vadd_devicecall(const void* in, void* scratch, u64 scratch_off,
                             u64 count, u32 tag, void* my_arena, u32 dst_rank,
-                            float addv, void* stream) {
+                            float addv, u32* err, void* stream) {
   hipLaunchKernelGGL(vadd_devicecall_kernel, dim3(1), dim3(64), 0,
                      (hipStream_t)stream, (const float*)in, (float*)scratch,
-                     scratch_off, count, tag, (char*)my_arena, dst_rank, addv);
+                     scratch_off, count, tag, (char*)my_arena, dst_rank, addv,
+                     err);
 }
 
 void launch_vadd_put(const void* in, u64 count, u32 tag, void* my_arena,
                      void* peer_arena, u32 me, u32 peer, u32 seg_bytes,
-                     float addv, void* stream) {
+                     float addv, u64 wait_ticks, u32* err, void* stream) {
   hipLaunchKernelGGL(vadd_put_kernel, dim3(1), dim3(64), 0,
                      (hipStream_t)stream, (const float*)in, count, tag,
                      (char*)my_arena, (char*)peer_arena, me, peer, seg_bytes,
-                     addv);
+                     addv, wait_ticks, err);
 }
 
 void launch_stream_drain(void* out, u64 max_elems, u32 nseg, void* my_arena,
