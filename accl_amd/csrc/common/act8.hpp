@@ -42,6 +42,12 @@ ACCL_HD inline int exponent_of(u32 largest) {
   return e < -126 ? -126 : e;
 }
 
+// The exponent by which float16 products take a group. Values that came from
+// float16 have at most 9 and are exact in it; a group beyond that is taken as
+// lost, since what it holds would overflow.
+constexpr int F16_MOST = 9;
+ACCL_HD inline int exponent_in_f16(int e) { return e > F16_MOST ? LOST : e; }
+
 // 1 / 2^e, and 0 where the group is lost (-126 <= e <= 121 otherwise)
 ACCL_HD inline float step_inverse(int e) {
   return e == LOST ? 0.0f : bits_float(u32(127 - e) << 23);

@@ -183,6 +183,7 @@ void host_act8_weight_grad(const WeightGradArgs& a) {
       const signed char* exps = a.exps + i64(m) * a.exps_stride;
       for (u64 k = 0; k < a.width; ++k) {
         int e = exps[k / act8::GROUP];
+        if (a.dtype == DataType::float16) e = act8::exponent_in_f16(e);
         sums[k] += g * (e == act8::LOST
                             ? double(NAN)
                             : double(float(codes[k]) * act8::step(e)));

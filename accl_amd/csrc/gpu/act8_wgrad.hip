@@ -21,6 +21,7 @@
 // code: 56 x 208 x 355 fp32 took 28 us when stores of whole and of cut groups of
 // columns stood unrolled behind the sums, and takes 14.5.
 #include <hip/hip_runtime.h>
+#include <type_traits>
 #include "../common/act8.hpp"
 #include "../common/tensor_ops.hpp"
 #include "ops_device.hpp"
@@ -58,7 +59,8 @@ __device__ inline f32x4 multiply(const Frag& a, const Frag& b, f32x4 c,
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.f, b.f, c, 0, 0, 0);
 }
 
-// two values as the matrix instructions take them; both are exact
+// Two values as the matrix instructions take them. Both are exact, in float16
+// because its exponents were bounded (exponent_in).
 __device__ inline u32 pack2(float lo, float hi, bf16) {
   return __builtin_amdgcn_perm(act8::float_bits(hi), act8::float_bits(lo),
                                0x07060302);
@@ -68,6 +70,11 @@ __device__ inline u32 pack2(float lo, float hi, fp16) {
   u32 w;
   __builtin_memcpy(&w, &v, 4);
   return w;
+}
+
+__device__ inline int exponent_in(int e, bf16) { return e; }
+__device__ inline int exponent_in(int e, fp16) {
+  return act8::exponent_in_f16(e);
 }
 
 // x as bfloat16 terms, the first ones cut short, so that they add up to x and
@@ -252,7 +259,9 @@ __global__ void __launch_bounds__(256, 2) ACCL_BESIDE_ENGINE
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g)
       scales[odd][wave * 2 + (GROUPS == 2 ? g : lane / 32)][lane % DEPTH] =
-          m0 + lane % DEPTH < m_end ? u16((exps[g] + 127) << 7) : u16(0);
+          m0 + lane % DEPTH < m_end
+              ? u16((exponent_in(exps[g], E()) + 127) << 7)
+              : u16(0);
   };
 
   // ---- decode: rows 8 quarter .. + 7 of a step
@@ -534,12 +543,13 @@ __global__ void __launch_bounds__(256) column_kernel(WeightGradArgs a) {
   const u32 lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const u64 n = u64(blockIdx.x) * 64 + lane;
   const i64 k = blockIdx.y;
+  using In = std::conditional_t<std::is_same_v<T, fp16>, fp16, bf16>;
   float v = 0.0f;
   if (n < a.outputs)
     for (u64 m = wave; m < a.rows; m += 4)
       v += float(((const T*)a.grad)[i64(m) * a.grad_stride + i64(n)]) *
            (float(a.codes[i64(m) * a.codes_stride + k]) *
-            act8::step(a.exps[i64(m) * a.exps_stride]));
+            act8::step(exponent_in(a.exps[i64(m) * a.exps_stride], In())));
   part[wave][lane] = v;
   __syncthreads();
   if (wave == 0 && n < a.outputs) {

@@ -312,7 +312,9 @@ class Act8:
     -127..127. A group that holds an infinity or a NaN has e = -128 and codes
     of zero, and stands for NaN.
 
-    codes: int8 [*, width]; exponents: int8 [*, groups]; dtype: of the values.
+    codes: int8 [*, width]; exponents: int8 [*, groups]; dtype: of the values
+    that were packed. Those of float16 have exponents of at most 9;
+    :func:`act8_weight_grad` takes a group beyond that as one that holds none.
     Both tensors are plain data: they can be sliced along rows, moved, or
     gathered over ranks at half the bytes of the values.
     """
