@@ -22,6 +22,8 @@ refused). A gradient has the same bits in every run. A persistent engine may be
 live on the same GPU: no kernel here needs more of a compute unit than the
 engine leaves.
 """
+import contextlib
+
 import torch
 
 from . import _core
@@ -541,6 +543,12 @@ def _gathered(t, group):
     return whole
 
 
+def _own_types(device):
+    """Products of operands whose type is settled, whatever autocast asks."""
+    return torch.autocast(device.type, enabled=False) \
+        if torch.is_autocast_enabled(device.type) else contextlib.nullcontext()
+
+
 def _product(x, weight, group):
     whole = x if group is None else _gathered(x, group)
     y = whole.reshape(-1, whole.size(-1)) @ weight.t()
@@ -556,18 +564,19 @@ class _Linear(torch.autograd.Function):
             ctx.save_for_backward(weight, kept.codes, kept.exponents)
         else:
             ctx.save_for_backward(weight)
-        ctx.group = group
+        ctx.of = (x.dtype, group)
         return _product(x, weight, group)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         weight, *kept = ctx.saved_tensors
-        group = ctx.group
+        dtype, group = ctx.of
         d_x = d_weight = None
         if ctx.needs_input_grad[0]:
-            d_x = (grad.reshape(-1, grad.size(-1)) @ weight).view(
-                *grad.shape[:-1], weight.size(1))
+            with _own_types(grad.device):
+                d_x = (grad.reshape(-1, grad.size(-1)) @ weight).view(
+                    *grad.shape[:-1], weight.size(1))
             if group is not None:
                 import torch.distributed as dist
                 whole = d_x
@@ -578,13 +587,14 @@ class _Linear(torch.autograd.Function):
         if ctx.needs_input_grad[1]:
             if group is not None:
                 kept = [_gathered(t, group) for t in kept]
-            d_weight = act8_weight_grad(grad, Act8(*kept, grad.dtype))
+            d_weight = act8_weight_grad(grad, Act8(*kept, dtype))
         return d_x, d_weight, None
 
 
 def act8_linear(x, weight, group=None):
     """``x @ weight.t()``, differentiable, with x kept in 8 bits for weight's
-    gradient. x: [*, width], weight: [outputs, width], of one type.
+    gradient. x: [*, width], weight: [outputs, width], of one type; under
+    autocast both are cast to its type first, as for a product of torch's.
 
     With a process group, x is this rank's part of a sequence (the same shape
     on every rank, at least two dimensions, split along the first): it is
@@ -593,6 +603,9 @@ def act8_linear(x, weight, group=None):
     """
     _value("x", x)
     _value("weight", weight)
+    if torch.is_autocast_enabled(x.device.type):
+        dtype = torch.get_autocast_dtype(x.device.type)
+        x, weight = x.to(dtype), weight.to(dtype)
     if weight.dtype != x.dtype:
         raise TypeError(f"x is {x.dtype}, weight {weight.dtype}")
     if weight.dim() != 2 or x.dim() < 1 or x.size(-1) != weight.size(1):
@@ -601,6 +614,8 @@ def act8_linear(x, weight, group=None):
     if group is not None and x.dim() < 2:
         raise ValueError("act8_linear: with a group, x needs two dimensions")
     _together(x, weight)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
-        return _capturable(_Linear.apply(x, weight, group))
-    return _product(x, weight, group)
+    with _own_types(x.device):
+        if torch.is_grad_enabled() and (x.requires_grad or
+                                        weight.requires_grad):
+            return _capturable(_Linear.apply(x, weight, group))
+        return _product(x, weight, group)
