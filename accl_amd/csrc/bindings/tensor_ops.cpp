@@ -79,13 +79,13 @@ void register_tensor_ops(py::module_& m) {
           else ops::gpu_gradient(a, (void*)stream);
         });
   m.def("ops_sum_rows",
-        [](i64 stream, u64 ids, u32 ids_dtype, u64 tokens, u64 rows, u64 width,
-           float scale, u64 src, i64 src_stride, u32 src_dtype, u64 dst,
-           i64 dst_stride, u32 dst_dtype, u64 ids_out, u64 count_out,
-           u64 workspace, u64 workspace_bytes) {
-          auto a = embedding_args(ids, ids_dtype, tokens, 0, rows, width,
-                                  scale, src, src_stride, src_dtype, dst,
-                                  dst_stride, dst_dtype);
+        [](i64 stream, u64 ids, u32 ids_dtype, u64 tokens, i64 first_row,
+           u64 rows, u64 width, float scale, u64 src, i64 src_stride,
+           u32 src_dtype, u64 dst, i64 dst_stride, u32 dst_dtype, u64 ids_out,
+           u64 count_out, u64 workspace, u64 workspace_bytes) {
+          auto a = embedding_args(ids, ids_dtype, tokens, first_row, rows,
+                                  width, scale, src, src_stride, src_dtype,
+                                  dst, dst_stride, dst_dtype);
           a.ids_out = (void*)ids_out;
           a.count_out = (i64*)count_out;
           a.workspace = (void*)workspace;

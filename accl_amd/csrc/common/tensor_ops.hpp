@@ -30,7 +30,8 @@ struct EmbeddingArgs {
   i64 dst_stride = 0;
   DataType dst_dtype = DataType::float32;
   bool accumulate = false;      // gradient: add to what dst holds
-  void* ids_out = nullptr;      // sum_rows: [tokens], type of ids
+  void* ids_out = nullptr;      // sum_rows: [tokens], rows as ids have them
+                                // less first_row, in the type of ids
   i64* count_out = nullptr;     // sum_rows: [1]
   void* workspace = nullptr;
   u64 workspace_bytes = 0;

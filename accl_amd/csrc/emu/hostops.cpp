@@ -89,9 +89,8 @@ void host_sum_rows(const EmbeddingArgs& a) {
     for (u64 c = 0; c < a.width; ++c)
       store_from_f64(a.dst, u64(i64(count) * a.dst_stride) + c, a.dst_dtype,
                      sums[c] * double(a.scale));
-    i64 id = r + a.first_row;
-    if (a.ids_dtype == DataType::int64) ((i64*)a.ids_out)[count] = id;
-    else ((i32*)a.ids_out)[count] = i32(id);
+    if (a.ids_dtype == DataType::int64) ((i64*)a.ids_out)[count] = r;
+    else ((i32*)a.ids_out)[count] = i32(r);
     j = end;
   }
   for (u64 i = count; i < a.tokens; ++i) {

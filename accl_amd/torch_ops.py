@@ -188,8 +188,8 @@ class _Embedding(torch.autograd.Function):
         if not sparse:
             return (None, embedding_grad(grad, ids, rows, scale, first_row,
                                          dtype=dtype), None, None, None)
-        at = ids.reshape(-1) - first_row if first_row else ids.reshape(-1)
-        found, sums, count = sum_rows(at, grad.reshape(-1, width), rows, scale)
+        found, sums, count = _sum_rows(
+            ids.reshape(-1), grad.reshape(-1, width), rows, scale, first_row)
         n = int(count)
         return (None, torch.sparse_coo_tensor(
             found[:n].long()[None], sums[:n].to(dtype), (rows, width),
@@ -286,6 +286,11 @@ def sum_rows(ids, values, rows, scale=1.0):
     if ids.dim() != 1 or values.dim() != 2 or values.size(0) != ids.size(0):
         raise ValueError(f"ids [n] and values [n, width] are needed, not "
                          f"{tuple(ids.shape)} and {tuple(values.shape)}")
+    return _sum_rows(ids, values, rows, scale, 0)
+
+
+def _sum_rows(ids, values, rows, scale, first_row):
+    """sum_rows of ``ids - first_row``, which may have more bits than ids."""
     n, width = values.shape
     index = _together(values, ids)
     ids = ids.contiguous()
@@ -296,8 +301,9 @@ def sum_rows(ids, values, rows, scale=1.0):
     size = 0 if index < 0 else _core.ops_gradient_workspace(
         n, rows, width, True)
     ws = _workspace(size, ids.device)
-    _run(index, _core.ops_sum_rows, ids.data_ptr(), _CODE[ids.dtype], n, rows,
-         width, scale, values.data_ptr(), stride, _CODE[values.dtype], sums.data_ptr(), width, _CODE[sums.dtype],
+    _run(index, _core.ops_sum_rows, ids.data_ptr(), _CODE[ids.dtype], n,
+         first_row, rows, width, scale, values.data_ptr(), stride,
+         _CODE[values.dtype], sums.data_ptr(), width, _CODE[sums.dtype],
          found.data_ptr(), count.data_ptr(), ws.data_ptr() if size else 0,
          size)
     return found, sums, count

@@ -1,0 +1,50 @@
+"""Derivatives of accl_amd.torch_ops where they are easily lost: tokens far from
+a shard, tensors without elements, forward mode, captures."""
+import pytest
+import torch
+
+from accl_amd import torch_ops as ops
+
+# Other tests fork this process: a pool of threads, which a fork does not
+# take along, must not have been started by then.
+torch.set_num_threads(1)
+
+_NEEDS = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(),
+                                              reason="no HIP GPU")]
+DEVICES = ["cpu", pytest.param("cuda", marks=_NEEDS)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+@pytest.mark.parametrize("tokens", [3, 300, 5000])
+@pytest.mark.parametrize("first", [2 ** 32 + 5, 2 ** 31, -2 ** 31, 2 ** 62])
+def test_shard_far_from_the_tokens(device, index, tokens, first):
+    """No token of a 32-bit type is in such a shard, though a difference in 32
+    bits would be: zeros, and no gradient, dense or sparse."""
+    ids = torch.arange(tokens, device=device, dtype=index).remainder(8) + 5
+    w = torch.ones(64, 3, device=device)
+    for sparse in (False, True):
+        leaf = w.clone().requires_grad_()
+        out = ops.embedding(ids, leaf, first_row=first, sparse=sparse)
+        assert not out.any()
+        out.backward(torch.ones_like(out))
+        assert leaf.grad.is_sparse == sparse
+        assert not leaf.grad.to_dense().any()
+        if sparse:
+            assert leaf.grad._nnz() == 0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("tokens", [4, 300, 5000])
+@pytest.mark.parametrize("first", [2 ** 40, -7, 1000])
+def test_sparse_gradient_of_a_shard(device, tokens, first):
+    """The touched rows, counted from the shard's first."""
+    ids = torch.arange(tokens, device=device).remainder(20) * 3 + first - 6
+    up = torch.ones(tokens, 5, device=device)
+    leaf = torch.zeros(31, 5, device=device).requires_grad_()
+    ops.embedding(ids, leaf, 2.0, first, sparse=True).backward(up)
+    at = (ids - first).cpu()
+    here = at[(at >= 0) & (at < 31)]
+    want = torch.bincount(here, minlength=31).float() * 2
+    assert leaf.grad._indices()[0].tolist() == here.unique().tolist()
+    assert torch.equal(leaf.grad.to_dense().cpu(), want[:, None].expand(31, 5))
