@@ -73,14 +73,18 @@ def _together(first, *others):
     return index
 
 
+def _matrix(t):
+    """t as a matrix of its last axis, also where that has no elements."""
+    return t.reshape(t.shape[:-1].numel(), t.size(-1))
+
+
 def _rows(t, width):
     """t as [rows, width] with neighbouring columns, and the distance of its
     rows: a view where its strides allow one, else a copy."""
     if t.dim() == 2 and t.is_contiguous():
         return t, width
     if t.dim() != 2 or (t.stride(1) != 1 and width > 1) or t.stride(0) < width:
-        t = t.reshape(-1, width) if width else t.reshape(
-            t.shape[:-1].numel(), 0)
+        t = _matrix(t)
         if (width > 1 and t.stride(1) != 1) or \
                 (t.size(0) > 1 and t.stride(0) < width):
             t = t.contiguous()
@@ -189,7 +193,7 @@ class _Embedding(torch.autograd.Function):
             return (None, embedding_grad(grad, ids, rows, scale, first_row,
                                          dtype=dtype), None, None, None)
         found, sums, count = _sum_rows(
-            ids.reshape(-1), grad.reshape(-1, width), rows, scale, first_row)
+            ids.reshape(-1), _matrix(grad), rows, scale, first_row)
         n = int(count)
         return (None, torch.sparse_coo_tensor(
             found[:n].long()[None], sums[:n].to(dtype), (rows, width),
@@ -557,7 +561,7 @@ def _own_types(device):
 
 def _product(x, weight, group):
     whole = x if group is None else _gathered(x, group)
-    y = whole.reshape(-1, whole.size(-1)) @ weight.t()
+    y = _matrix(whole) @ weight.t()
     return y.view(*whole.shape[:-1], weight.size(0))
 
 
@@ -581,7 +585,7 @@ class _Linear(torch.autograd.Function):
         d_x = d_weight = None
         if ctx.needs_input_grad[0]:
             with _own_types(grad.device):
-                d_x = (grad.reshape(-1, grad.size(-1)) @ weight).view(
+                d_x = (_matrix(grad) @ weight).view(
                     *grad.shape[:-1], weight.size(1))
             if group is not None:
                 import torch.distributed as dist

@@ -48,3 +48,45 @@ def test_sparse_gradient_of_a_shard(device, tokens, first):
     want = torch.bincount(here, minlength=31).float() * 2
     assert leaf.grad._indices()[0].tolist() == here.unique().tolist()
     assert torch.equal(leaf.grad.to_dense().cpu(), want[:, None].expand(31, 5))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("sparse", [False, True])
+@pytest.mark.parametrize("shape", [(3,), (2, 3), (0,), (0, 3), ()])
+@pytest.mark.parametrize("rows,width", [(10, 0), (0, 4), (10, 4)])
+def test_embedding_without_elements(device, sparse, shape, rows, width):
+    weight = torch.ones(rows, width, device=device).requires_grad_()
+    ids = torch.ones(shape, dtype=torch.int64, device=device)
+    out = ops.embedding(ids, weight, sparse=sparse)
+    assert out.shape == (*shape, width)
+    out.backward(torch.ones_like(out))
+    want = torch.zeros(rows, width)
+    want[1:2] = ids.numel()
+    assert torch.equal(weight.grad.to_dense().cpu(), want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lead", [(5,), (2, 3), (0,), (0, 3), ()])
+@pytest.mark.parametrize("outputs,width", [(24, 0), (0, 40), (0, 0), (24, 40)])
+def test_linear_without_elements(device, lead, outputs, width):
+    x = torch.ones(*lead, width, device=device).requires_grad_()
+    w = torch.ones(outputs, width, device=device).requires_grad_()
+    with torch.no_grad():
+        assert ops.act8_linear(x, w).shape == (*lead, outputs)
+    y = ops.act8_linear(x, w)
+    assert y.shape == (*lead, outputs) and (y == width).all()
+    y.backward(torch.ones_like(y))
+    assert x.grad.shape == x.shape and (x.grad == outputs).all()
+    assert w.grad.shape == w.shape
+    assert (w.grad == torch.Size(lead).numel()).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lead", [(5,), (0,), (0, 3)])
+@pytest.mark.parametrize("width", [0, 6])
+def test_swiglu_without_elements(device, lead, width):
+    x = torch.ones(*lead, 2 * width, device=device).requires_grad_()
+    y = ops.act8_swiglu(x)
+    assert y.shape == (*lead, width)
+    y.backward(torch.ones_like(y))
+    assert x.grad.shape == x.shape and x.grad.isfinite().all()
