@@ -25,6 +25,7 @@ engine leaves.
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _core
 from .accl import DataType, _torch_dtype_map
@@ -42,7 +43,7 @@ _CODE = {t: int(d) for d, t in _torch_dtype_map().items()}
 
 
 # ------------------------------------------------------------------ checks
-def _value(name, t):
+def _value(name, t, tangent=False):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: a tensor is needed, not {type(t).__name__}")
     if t.layout is not torch.strided:
@@ -50,6 +51,11 @@ def _value(name, t):
     if t.dtype not in _VALUES:
         raise TypeError(f"{name}: float32, bfloat16 or float16 are supported, "
                         f"not {t.dtype}")
+    # without a tangent a result would read as a derivative of zero
+    if not tangent and forward_ad._current_level >= 0 and \
+            forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeError(f"{name}: forward-mode derivatives are not "
+                           f"supported")
     return t
 
 
@@ -611,8 +617,8 @@ def act8_linear(x, weight, group=None):
     gathered before the product, x's gradient is reduced and scattered, and
     what the backward pass gathers again are the 8-bit codes.
     """
-    _value("x", x)
-    _value("weight", weight)
+    _value("x", x, tangent=True)
+    _value("weight", weight, tangent=True)
     if torch.is_autocast_enabled(x.device.type):
         dtype = torch.get_autocast_dtype(x.device.type)
         x, weight = x.to(dtype), weight.to(dtype)

@@ -90,3 +90,49 @@ def test_swiglu_without_elements(device, lead, width):
     assert y.shape == (*lead, width)
     y.backward(torch.ones_like(y))
     assert x.grad.shape == x.shape and x.grad.isfinite().all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("trained", [False, True])
+def test_forward_mode_is_refused(device, trained):
+    """A result without a tangent would read as a derivative of zero."""
+    import torch.autograd.forward_ad as fwd
+    ids = torch.tensor([1, 2], device=device)
+    x = torch.ones(2, 8, device=device).requires_grad_(trained)
+    kept = ops.act8_pack(torch.ones(2, 8, device=device))
+    two = ops.act8_swiglu_forward(torch.ones(2, 8, device=device))[1]
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for call in (lambda: ops.embedding(ids, dual),
+                     lambda: ops.embedding(ids, dual, sparse=True),
+                     lambda: ops.embedding_grad(dual, ids, 4),
+                     lambda: ops.sum_rows(ids, dual, 4),
+                     lambda: ops.act8_pack(dual),
+                     lambda: ops.act8_weight_grad(dual, kept),
+                     lambda: ops.act8_swiglu(dual),
+                     lambda: ops.act8_swiglu_forward(dual),
+                     lambda: ops.act8_swiglu_grad(dual[:, :4], two)):
+            with pytest.raises(RuntimeError, match="forward"):
+                call()
+        out = torch.zeros(4, 8, device=device)
+        with pytest.raises(RuntimeError, match="forward"):
+            ops.embedding_grad(x.detach(), ids, 4,
+                               out=fwd.make_dual(out, torch.ones_like(out)))
+        # tensors without a tangent are as ever
+        assert ops.embedding(ids, x).shape == (2, 8)
+        ops.act8_swiglu(x)
+    ops.embedding(ids, dual)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_forward_mode_of_the_product(device):
+    """With operands that are not trained act8_linear is torch's product, and
+    has its tangent."""
+    import torch.autograd.forward_ad as fwd
+    x, w = torch.ones(2, 8, device=device), torch.ones(3, 8, device=device)
+    with fwd.dual_level():
+        y = ops.act8_linear(fwd.make_dual(x, 2 * x), w)
+        assert (fwd.unpack_dual(y).tangent == 16).all()
+        with pytest.raises(RuntimeError):
+            ops.act8_linear(fwd.make_dual(x, 2 * x),
+                            w.clone().requires_grad_())
