@@ -60,7 +60,7 @@ __device__ inline f32x4 multiply(const Frag& a, const Frag& b, f32x4 c,
 }
 
 // Two values as the matrix instructions take them. Both are exact, in float16
-// because its exponents were bounded (exponent_in).
+// because its exponents were bounded (scale_bits).
 __device__ inline u32 pack2(float lo, float hi, bf16) {
   return __builtin_amdgcn_perm(act8::float_bits(hi), act8::float_bits(lo),
                                0x07060302);
@@ -72,9 +72,12 @@ __device__ inline u32 pack2(float lo, float hi, fp16) {
   return w;
 }
 
-__device__ inline int exponent_in(int e, bf16) { return e; }
-__device__ inline int exponent_in(int e, fp16) {
-  return act8::exponent_in_f16(e);
+// 2^e as bfloat16, NaN where the group holds none or one that overflows
+__device__ inline u16 scale_bits(int e, bf16) {
+  return e == act8::LOST ? u16(0x7FC0) : u16((e + 127) << 7);
+}
+__device__ inline u16 scale_bits(int e, fp16) {
+  return scale_bits(act8::exponent_in_f16(e), bf16());
 }
 
 // x as bfloat16 terms, the first ones cut short, so that they add up to x and
@@ -259,9 +262,7 @@ __global__ void __launch_bounds__(256, 2) ACCL_BESIDE_ENGINE
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g)
       scales[odd][wave * 2 + (GROUPS == 2 ? g : lane / 32)][lane % DEPTH] =
-          m0 + lane % DEPTH < m_end
-              ? u16((exponent_in(exps[g], E()) + 127) << 7)
-              : u16(0);
+          m0 + lane % DEPTH < m_end ? scale_bits(exps[g], E()) : u16(0);
   };
 
   // ---- decode: rows 8 quarter .. + 7 of a step
@@ -549,7 +550,8 @@ __global__ void __launch_bounds__(256) column_kernel(WeightGradArgs a) {
     for (u64 m = wave; m < a.rows; m += 4)
       v += float(((const T*)a.grad)[i64(m) * a.grad_stride + i64(n)]) *
            (float(a.codes[i64(m) * a.codes_stride + k]) *
-            act8::step(exponent_in(a.exps[i64(m) * a.exps_stride], In())));
+            act8::bits_float(
+                u32(scale_bits(a.exps[i64(m) * a.exps_stride], In())) << 16));
   part[wave][lane] = v;
   __syncthreads();
   if (wave == 0 && n < a.outputs) {
