@@ -17,8 +17,8 @@ Values are float32, bfloat16 or float16, sums are held in 32 bits, and every
 result is rounded once. No function waits for the GPU or keeps anything
 between calls: results and workspaces come from torch's allocator, so calls
 can run on several streams at once and be captured into graphs (forward and
-backward pass; a capture over a parameter of which an eager graph lives is
-refused). A gradient has the same bits in every run. A persistent engine may be
+backward pass; a capture over a parameter whose gradient belongs to the default
+stream is refused). A gradient has the same bits in every run. A persistent engine may be
 live on the same GPU: no kernel here needs more of a compute unit than the
 engine leaves.
 """
@@ -134,9 +134,10 @@ def _apart(name, out, *operands):
 
 def _capturable(y):
     """Marks the gradient accumulators that y's graph holds with the stream
-    they belong to, and refuses a capture over one of another stream: a
-    backward pass that is captured while an eager graph of the same parameter
-    lives ends the process."""
+    they were first met on, and refuses a capture over one of the default
+    stream: a backward pass that is captured there ends the process, since the
+    default stream cannot take part in a capture. One of another stream can,
+    as after the usual steps on a side stream before a capture."""
     if y.is_cuda:
         stream = torch._C._cuda_getCurrentRawStream(y.device.index)
         capturing = torch.cuda.is_current_stream_capturing()
@@ -144,10 +145,13 @@ def _capturable(y):
             if node is not None and \
                     node.name() == "torch::autograd::AccumulateGrad":
                 made = node.metadata.setdefault("accl_stream", stream)
-                if capturing and made != stream:
+                if capturing and made == 0:
                     raise RuntimeError(
-                        "accl_amd: an eager graph of a parameter of this call "
-                        "is alive; drop its results before the capture, or "
+                        "accl_amd: the gradient of a parameter of this call "
+                        "belongs to the default stream, since an eager graph "
+                        "of it is alive, or DDP or a hook keeps it so. Drop "
+                        "the graph's results before the capture, run eager "
+                        "steps (and construct DDP) on a side stream, or "
                         "capture with parameter.detach().requires_grad_()")
     return y
 

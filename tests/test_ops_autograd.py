@@ -136,3 +136,47 @@ def test_forward_mode_of_the_product(device):
         with pytest.raises(RuntimeError):
             ops.act8_linear(fwd.make_dual(x, 2 * x),
                             w.clone().requires_grad_())
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(not torch.cuda.is_available(), reason="no HIP GPU")
+@pytest.mark.parametrize("operator", ["embedding", "linear"])
+@pytest.mark.parametrize("held", [False, True])
+def test_capture_after_steps_on_a_side_stream(operator, held):
+    """Eager steps on a side stream, whose results still live, then a capture of
+    forward and backward pass on another one, replayed over new inputs. With
+    `held` the parameter's accumulator is kept as DDP keeps it."""
+    g = torch.Generator().manual_seed(0)
+    w = torch.randn(50, 64, generator=g).cuda().requires_grad_()
+    x = torch.randn(10, 64, generator=g).cuda()
+    ids = torch.randint(0, 50, (10,), generator=g).cuda()
+
+    def step(weight):
+        y = ops.embedding(ids, weight, 2.0) if operator == "embedding" else \
+            ops.act8_linear(x, weight)
+        y.backward(y.detach())
+        return y
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        if held:
+            kept = w.view_as(w).grad_fn.next_functions[0][0]
+        for _ in range(3):
+            w.grad = None
+            alive = step(w)
+    torch.cuda.current_stream().wait_stream(side)
+    w.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = step(w)
+    for seed in range(3):
+        g.manual_seed(seed)
+        with torch.no_grad():
+            x.copy_(torch.randn(10, 64, generator=g).cuda())
+            ids.copy_(torch.randint(0, 50, (10,), generator=g).cuda())
+        graph.replay()
+        torch.cuda.synchronize()
+        leaf = w.detach().requires_grad_()
+        assert torch.equal(step(leaf), y)
+        assert torch.equal(leaf.grad, w.grad)
+    assert alive.shape == y.shape and (not held or kept is not None)
