@@ -119,6 +119,19 @@ def _range(t):
         1 + sum((n - 1) * d for n, d in zip(t.shape, t.stride()))) - 1
 
 
+def _side_by_side(a, b):
+    """Whether rows of a and b, equally far apart, take different columns of one
+    buffer."""
+    if a.dim() != 2 or b.dim() != 2:
+        return False
+    row = a.stride(0) * a.element_size()
+    a_width, b_width = (t.size(1) * t.element_size() for t in (a, b))
+    if b.stride(0) * b.element_size() != row or max(a_width, b_width) > row or \
+            any(t.size(1) > 1 and t.stride(1) != 1 for t in (a, b)):
+        return False
+    return a_width <= (b.data_ptr() - a.data_ptr()) % row <= row - b_width
+
+
 def _apart(name, out, *operands):
     """An `out` that shares memory with an operand would be read and written
     at once."""
@@ -127,7 +140,7 @@ def _apart(name, out, *operands):
         for t in operands:
             if t.numel():
                 a, b = _range(t)
-                if a <= last and first <= b:
+                if a <= last and first <= b and not _side_by_side(out, t):
                     raise ValueError(
                         f"{name}: out shares its memory with an operand")
 

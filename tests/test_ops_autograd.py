@@ -180,3 +180,49 @@ def test_capture_after_steps_on_a_side_stream(operator, held):
         assert torch.equal(step(leaf), y)
         assert torch.equal(leaf.grad, w.grad)
     assert alive.shape == y.shape and (not held or kept is not None)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_out_between_the_columns_of_an_operand(device, dtype):
+    """Columns of one buffer, side by side: rows of out lie between rows of the
+    operand, and share no element with them."""
+    g = torch.Generator().manual_seed(0)
+    room = torch.randn(40, 48, generator=g).to(dtype).to(device)
+    grad, out = room[:24, :19], room[:, 19:38]
+    ids = torch.arange(24, device=device).remainder(7)
+    want = ops.embedding_grad(grad.clone(), ids, 40, out=out.clone())
+    before = room.clone()
+    assert ops.embedding_grad(grad, ids, 40, out=out) is out
+    assert torch.equal(out, want)
+    assert torch.equal(room[:, :19], before[:, :19])
+    assert torch.equal(room[:, 38:], before[:, 38:])
+    # behind the columns of out, and round the end of a row
+    ops.embedding_grad(room[:24, 29:48], ids, 40, out=room[:, 5:24])
+    ops.embedding_grad(room.view(-1)[43:43 + 48 * 24].view(24, 48)[:, :8], ids,
+                       40, out=room[:, 3:11])
+    kept = ops.act8_pack(torch.ones(40, 19, device=device, dtype=dtype))
+    ops.act8_weight_grad(room[:, :24], kept, out=room[:24, 24:43])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_out_that_shares_elements(device):
+    room = torch.zeros(40, 48, device=device)
+    ids = torch.arange(24, device=device).remainder(7)
+    flat = room.view(-1)
+    for grad, out in [
+            (room[:24, :19], room[:, 18:37]),
+            (room[:24, 20:39], room[:, 20:39]),
+            (room[:24, 20:39], room[:, 2:21]),
+            # a row that goes on at the beginning of the next
+            (flat[40:40 + 48 * 24].view(24, 48)[:, :9], room[:, :9]),
+            (room[:24, :9], flat[40:40 + 48 * 39].view(39, 48)[:, :9]),
+            # rows of another distance
+            (flat[19:19 + 24 * 19].view(24, 19), room[:, 19:38]),
+            (room.t()[:24, :19], room[:, 19:38])]:
+        with pytest.raises(ValueError, match="shares"):
+            ops.embedding_grad(grad, ids[:len(grad)], out.size(0), out=out)
+    with pytest.raises(ValueError, match="shares"):
+        ops.embedding_grad(torch.zeros(480, 5, device=device),
+                           room.view(torch.int32).view(-1)[:480],
+                           40, out=room[:, 7:12])
