@@ -137,9 +137,27 @@ __global__ void __launch_bounds__(256) unpack_kernel(Act8Args a) {
   }
 }
 
-// 1 / (1 + exp(-x)); the two fast operations are off by a few units of 2^-24
+// 1 / (1 + exp(-x)) for a result in T. For float32 it is off by at most 7 units of
+// 2^-24 of its size: two of the power, one each of its factor, their product and
+// the sum, two of the reciprocal. The factor is what rounding x log2(e) left, which
+// goes into the exponent: without it, as for the 16-bit types, the result is off
+// by up to |x| units more, of which their rounding shows none (and the gradient of
+// 8192 x 12288 bf16 takes 135 us instead of 141).
+template <class T>
 __device__ inline float logistic(float x) {
-  return __builtin_amdgcn_rcpf(1.0f + __expf(-x));
+  if constexpr (sizeof(T) == 2) {
+    return __builtin_amdgcn_rcpf(1.0f + __expf(-x));
+  } else {
+    // REST: log2(e) - LOG2E
+    constexpr float LOG2E = 0x1.715476p+0f, REST = 0x1.4ae0cp-26f;
+    constexpr float LN2 = 0x1.62e43p-1f;
+    const float v = __builtin_amdgcn_fmed3f(-x, -128.0f, 128.0f);
+    const float t = v * LOG2E;
+    const float left = __builtin_fmaf(v, REST, __builtin_fmaf(v, LOG2E, -t));
+    const float e =
+        __builtin_amdgcn_exp2f(t) * __builtin_fmaf(left, LN2, 1.0f);
+    return __builtin_amdgcn_rcpf(1.0f + e);
+  }
 }
 
 template <class T>
@@ -158,7 +176,7 @@ __global__ void __launch_bounds__(256) swiglu_kernel(Act8Args a) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       const float g = float(gate.e[i]);
-      y.e[i] = T(g * logistic(g) * float(up.e[i]));
+      y.e[i] = T(g * logistic<T>(g) * float(up.e[i]));
     }
     stream8((T*)a.y + i64(r) * a.y_stride + i64(at.c), at.n, y);
     signed char* codes = a.codes + i64(r) * a.codes_stride + i64(at.c);
@@ -189,7 +207,7 @@ __global__ void __launch_bounds__(256) swiglu_grad_kernel(Act8Args a) {
     load8((const T*)a.y + i64(r) * a.y_stride + i64(at.c), at.n, grad);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      const float d = float(grad.e[i]), s = logistic(gate[i]);
+      const float d = float(grad.e[i]), s = logistic<T>(gate[i]);
       d_gate.e[i] = T(d * up[i] * s * (1.0f + gate[i] * (1.0f - s)));
       d_up.e[i] = T(d * gate[i] * s);
     }

@@ -226,3 +226,27 @@ def test_out_that_shares_elements(device):
         ops.embedding_grad(torch.zeros(480, 5, device=device),
                            room.view(torch.int32).view(-1)[:480],
                            40, out=room[:, 7:12])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_gated_unit_of_large_gates(device):
+    """Both directions of gates far from zero, where the logistic function is a
+    power of e or one less such a power: off by 7 units of 2^-24, and by one for
+    each product behind it (two, and two more that the codes leave exact)."""
+    # multiples of 2^-1 below 127 of them: what is kept is exact
+    gate = torch.arange(-126, 127).remainder(127).sub(63).mul(0.5)
+    gate = torch.cat([gate, -gate]).clamp(-60, 60).view(-1, 1).expand(-1, 32)
+    gate = gate.contiguous()
+    gate[:, 0] = 63.5  # the group's unit
+    up = torch.ones_like(gate)
+    x = torch.cat([gate, up], 1)
+    y, kept = ops.act8_swiglu_forward(x.to(device))
+    assert torch.equal(ops.act8_unpack(kept).cpu(), x)
+    d = ops.act8_swiglu_grad(torch.ones_like(y), kept)
+    wide = gate.double()
+    sig = 1 / (1 + torch.exp(-wide))
+    exact = wide * sig
+    unit = 2.0 ** -24
+    assert ((y.cpu().double() - exact).abs() <= 9 * unit * exact.abs()).all()
+    assert ((d[:, 32:].cpu().double() - exact).abs()
+            <= 9 * unit * exact.abs()).all()
