@@ -72,12 +72,15 @@ __device__ inline u32 pack2(float lo, float hi, fp16) {
   return w;
 }
 
-// 2^e as bfloat16, NaN where the group holds none or one that overflows
-__device__ inline u16 scale_bits(int e, bf16) {
-  return e == act8::LOST ? u16(0x7FC0) : u16((e + 127) << 7);
+// 2^e as bfloat16, NaN where the group holds none (whose byte gives a number
+// above all others) or one that overflows
+__device__ inline u16 scale_bits(int e, u16 most) {
+  const u16 scale = u16((e + 127) << 7);
+  return scale > most ? u16(0x7FC0) : scale;
 }
+__device__ inline u16 scale_bits(int e, bf16) { return scale_bits(e, u16(0x7F00)); }
 __device__ inline u16 scale_bits(int e, fp16) {
-  return scale_bits(act8::exponent_in_f16(e), bf16());
+  return scale_bits(e, u16((act8::F16_MOST + 127) << 7));
 }
 
 // x as bfloat16 terms, the first ones cut short, so that they add up to x and
@@ -139,10 +142,6 @@ __device__ inline u32 here(u32 offset) {
   return offset;
 }
 
-// Four waves of at most 208 registers find room on a compute unit beside the
-// eight or twelve waves that a live engine keeps there.
-#define ACCL_BESIDE_ENGINE __attribute__((amdgpu_num_vgpr(104)))
-
 // The gradients as the matrix instructions take them: 16-bit values in rows of
 // a multiple of 8, at 16-byte addresses, so that they go to LDS without a stop
 // in registers. Float32 gradients have three planes of them.
@@ -158,7 +157,7 @@ struct Yes { __device__ constexpr operator bool() const { return true; } };
 // E: type of the matrix instructions; DEPTH: tokens between two barriers. With
 // `partial`, sums of this part of the tokens go there.
 template <class E, class O, int PLANES, int DEPTH>
-__global__ void __launch_bounds__(256, 2) ACCL_BESIDE_ENGINE
+__global__ void __launch_bounds__(256, 2)
     weight_grad_kernel(WeightGradArgs a, Grads grads, u32 tiles_n, u32 tiles_k,
                        u32 items, u64 part_rows, float* partial) {
   constexpr int STEPS = DEPTH / 32;
