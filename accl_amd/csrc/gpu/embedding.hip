@@ -171,7 +171,8 @@ static u32 fill_groups(u64 bytes, u32 shares) {
 
 // ----------------------------------------------------------------------- sort
 // Stable least-significant-digit radix sort of (row, place). Digits have at
-// most 9 bits, so that a vocabulary of 2^18 rows takes two passes. Up to 4096
+// most 9 bits, so that a vocabulary of fewer than 2^18 rows takes two passes
+// (tokens without a row have the number behind the last as theirs). Up to 4096
 // tokens are sorted by one workgroup in LDS, in one launch (a gradient of 2048
 // tokens took 25 us in tiles and 19 so, of 4096 28 and 27, of 8192, if allowed,
 // 36 and 43). More of them are cut in tiles: for each pass a histogram of each

@@ -18,9 +18,13 @@ result is rounded once. No function waits for the GPU or keeps anything
 between calls: results and workspaces come from torch's allocator, so calls
 can run on several streams at once and be captured into graphs (forward and
 backward pass; a capture over a parameter whose gradient belongs to the default
-stream is refused). A gradient has the same bits in every run. A persistent engine may be
-live on the same GPU: no kernel here needs more of a compute unit than the
-engine leaves.
+stream is refused). A gradient has the same bits in every run.
+
+A persistent engine may be live on the same GPU: its kernels leave these room.
+But they never end, and hold two of the four hardware queues that HIP deals a
+process's streams out to, so keep to the default stream beside an engine: work
+on a side stream may wait until the engine is closed, whoever launches it. What
+waits for the whole device (torch.cuda.synchronize, empty_cache) does wait.
 """
 import contextlib
 
