@@ -609,6 +609,10 @@ PYBIND11_MODULE(_core, m) {
            u32 tag, float addv) {
           auto* g = dynamic_cast<GpuDevice*>(a.backend());
           if (!g) throw accl_error("demo_vadd_devicecall: gpu backend only");
+          if (dst >= g->cfg().nranks || count > src.bytes() / sizeof(float) ||
+              count > scratch.bytes() / sizeof(float))
+            throw accl_error("demo_vadd_devicecall: no such rank, or more "
+                             "values than the buffers hold");
           run_demo("demo_vadd_devicecall", g, [&](u32* err, hipStream_t st) {
             launch_vadd_devicecall(
                 g->arena_local() + src.arena_offset(),
@@ -628,6 +632,9 @@ PYBIND11_MODULE(_core, m) {
            u32 wait_ms) {
           auto* g = dynamic_cast<GpuDevice*>(a.backend());
           if (!g) throw accl_error("demo_vadd_put: gpu backend only");
+          if (dst >= g->cfg().nranks || count > src.bytes() / sizeof(float))
+            throw accl_error("demo_vadd_put: no such rank, or more values than "
+                             "the buffer holds");
           u32 seg = g->cfg().stream_bytes < (32u << 10) ? g->cfg().stream_bytes
                                                         : (32u << 10);
           run_demo("demo_vadd_put", g, [&](u32* err, hipStream_t st) {

@@ -26,6 +26,24 @@ def test_needs_a_gpu_engine(demo):
         a.close()
 
 
+@pytest.mark.gpu
+@pytest.mark.skipif(not torch.cuda.is_available(), reason="no HIP GPU")
+def test_refuses_ranks_and_counts_that_are_not_there():
+    """On the host: neither call launches anything."""
+    a = A.ACCL(nranks=1, rank=0, backend="gpu", heap_bytes=64 << 20)
+    try:
+        s, t = (a.create_buffer(n, A.DataType.float32) for n in (16, 8))
+        for call in (lambda: core.demo_vadd_put(a._a, s, 16, 1),
+                     lambda: core.demo_vadd_put(a._a, s, 17, 0),
+                     lambda: core.demo_vadd_devicecall(a._a, s, s, 16, 1),
+                     lambda: core.demo_vadd_devicecall(a._a, s, t, 9, 0),
+                     lambda: core.demo_vadd_devicecall(a._a, t, s, 9, 0)):
+            with pytest.raises(RuntimeError, match="no such rank"):
+                call()
+    finally:
+        a.close()
+
+
 @pytest.mark.parametrize("rooms", [1, 4])
 @pytest.mark.parametrize("wait_ms", [0, 20])
 class TestPush:
