@@ -94,8 +94,13 @@ void EmuDevice::connect(const std::vector<std::vector<char>>& blobs) {
     int fd = -1;
     u64 t0 = wallclock_host_ns();
     for (;;) {
+      // an arena has its name before it has its size, and memory behind a
+      // file's end ends the process; the name may also be a former run's
       fd = shm_open(name.c_str(), O_RDWR, 0600);
-      if (fd >= 0) break;
+      struct stat st;
+      if (fd >= 0 && fstat(fd, &st) == 0 && u64(st.st_size) >= arena_bytes_)
+        break;
+      if (fd >= 0) close(fd);
       if (wallclock_host_ns() - t0 > 30ull * 1000000000)
         throw accl_error("emu: peer arena " + name + " never appeared");
       usleep(1000);
